@@ -30,9 +30,11 @@ void expect_beside(const Tensor &t, const Tensor &first, const char *what) {
 // -------------------------------------------------------------------- layer norm ----
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &features, const OptTensor &weight_,
+  // `x` is contiguous already: a copy made in here would be saved without its history, and gradients
+  // that are themselves differentiated would not reach the features.
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const OptTensor &weight_,
                         const OptTensor &bias_, double eps, bool keep) {
-    const Tensor x = features.contiguous(), weight = opt(weight_), bias = opt(bias_);
+    const Tensor weight = opt(weight_), bias = opt(bias_);
     const int type = feature_type(x, "layer_norm");
     const int64_t cols = x.size(-1), rows = cols ? x.numel() / cols : 0;
     Tensor y = at::empty_like(x), stats;  // (means, then 1 / deviations)
@@ -107,7 +109,7 @@ Tensor layer_norm(const Tensor &features, const OptTensor &weight, const OptTens
   for (const Tensor &t : {opt(weight), opt(bias)}) (void)f32(t);     // (type and layout)
   const bool keep = at::GradMode::is_enabled() &&
                     (wants_grad(features) || wants_grad(opt(weight)) || wants_grad(opt(bias)));
-  return LayerNorm::apply(features, weight, bias, eps, keep);
+  return LayerNorm::apply(features.contiguous(), weight, bias, eps, keep);
 }
 
 // --------------------------------------------------------------------- attention ----
