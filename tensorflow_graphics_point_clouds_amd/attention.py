@@ -74,6 +74,12 @@ def offset_buckets(num_buckets, max_offset, bidirectional=True, device="cuda"):
 
 def row_splits(point_cloud):
     """Row offsets of the clouds of a `PointCloud`, int32 [clouds + 1], for `packed_attention`; its
-    points have to be stored cloud after cloud."""
+    points have to be stored cloud after cloud (put into `point_cloud.get_cloud_order()`)."""
+    if point_cloud.get_cloud_order() is not None:
+        raise _lib.InvalidArgumentError("row_splits expects points that are stored cloud after cloud")
+    return _splits(point_cloud)
+
+
+def _splits(point_cloud):
     sizes = point_cloud.get_sizes().reshape(-1)
     return torch.nn.functional.pad(sizes.cumsum(0), (1, 0)).to(_I32)

@@ -311,8 +311,10 @@ class PointAttention(torch.nn.Module):
     `attention.packed_attention`, a 1x1 map back.  `num_key_heads` heads of keys and values are shared
     by the query heads; `attention_type` is the type of queries, keys and values.
 
-    The points are stored cloud after cloud.  With `queries` [clouds, num_features] those features
-    look at the clouds instead, one row each (the pooling of a network's end)."""
+    Points that are not stored cloud after cloud are put so for the attention, `positions` with them,
+    and their results back; `splits` are the row offsets of the clouds in that order.  With `queries`
+    [clouds, num_features] those features look at the clouds instead, one row each (the pooling of a
+    network's end)."""
 
     def __init__(self, num_features, num_heads, num_key_heads=None, relative_bias=None,
                  causal=False, attention_type=_F32, device="cuda", seed=0):
@@ -332,7 +334,11 @@ class PointAttention(torch.nn.Module):
     def forward(self, features, point_cloud, splits=None, positions=None, queries=None,
                 query_positions=None, return_sorted=False, return_padded=False):
         features = point_cloud.flatten_features(features)
-        splits = attention.row_splits(point_cloud) if splits is None else splits
+        order = point_cloud.get_cloud_order()
+        if order is not None:
+            features = features[order]
+            positions = None if positions is None else positions[order]
+        splits = attention._splits(point_cloud) if splits is None else splits
         clouds = splits.shape[0] - 1
         heads = lambda x, h: x.to(self._type).unflatten(1, (h, -1))
         rows, query_splits = features, splits
@@ -345,14 +351,17 @@ class PointAttention(torch.nn.Module):
         bias = self.relative_bias
         out = attention.packed_attention(
             heads(self.query(rows, plain), self._heads),
-            heads(self.key(features, point_cloud), self._key_heads),
-            heads(self.value(features, point_cloud), self._key_heads), query_splits, splits,
+            heads(self.key(features, plain), self._key_heads),
+            heads(self.value(features, plain), self._key_heads), query_splits, splits,
             causal=self._causal, bias_table=None if bias is None else bias.table,
             bias_buckets=None if bias is None else bias.buckets, query_positions=query_positions,
             key_positions=positions)
         out = self.out(out.flatten(1).to(rows.dtype), plain)
-        return out if queries is not None else point_cloud.format_output(out, return_sorted,
-                                                                         return_padded)
+        if queries is not None:
+            return out
+        if order is not None:
+            out = torch.empty_like(out).index_copy(0, order, out)
+        return point_cloud.format_output(out, return_sorted, return_padded)
 
 
 class _Rows:

@@ -156,9 +156,12 @@ class AttentionNet(torch.nn.Module):
             torch.nn.Linear(num_features, num_classes, device=device)])
 
     def forward(self, points, sizes=None, training=None, batch_ids=None, batch_size=None):
-        """points [B, V, 3] with `sizes` [B] (or [N, 3] with `batch_ids`, cloud after cloud) ->
+        """points [B, V, 3] with `sizes` [B] (or [N, 3] with `batch_ids`, in any order) ->
         logits [B, classes]."""
         cloud = pc.PointCloud(points, batch_ids=batch_ids, batch_size=batch_size, sizes=sizes)
+        order = cloud.get_cloud_order()
+        if order is not None:                          # once, not in every layer
+            cloud = pc.PointCloud(cloud._points[order], sizes=cloud.get_sizes().reshape(-1))
         splits = attention.row_splits(cloud)
         cells = torch.floor(cloud._points.detach() / self.cell_size).to(torch.int32)
         features = self.embed(cloud._points, cloud)

@@ -133,6 +133,8 @@ class PointCloud:
     def __init__(self, points, batch_ids=None, batch_size=None, sizes=None):
         points = torch.as_tensor(points, dtype=_F32)
         dev = points.device
+        # points given with their ids may be stored in any order (`get_cloud_order`)
+        self._cloud_order = () if batch_ids is not None and points.dim() == 2 else None
         self._sizes = None if sizes is None else torch.as_tensor(sizes, dtype=_I32, device=dev)
         self._batch_shape = None
         if points.dim() < 2:
@@ -195,6 +197,16 @@ class PointCloud:
             if self._batch_shape is not None:
                 self._sizes = self._sizes.reshape(self._batch_shape)
         return self._sizes
+
+    def get_cloud_order(self):
+        """None where the points are stored cloud after cloud, else the order that puts them so (int64
+        [N], stable).  Looked up on the first call if the points came with batch ids (which waits
+        for the device); no counterpart in the reference."""
+        if isinstance(self._cloud_order, tuple):
+            ids = self._batch_ids
+            sorted_already = bool((ids[1:] >= ids[:-1]).all())
+            self._cloud_order = None if sorted_already else torch.argsort(ids.long(), stable=True)
+        return self._cloud_order
 
     def set_batch_shape(self, batch_shape):
         """PointCloud.py:262-290."""

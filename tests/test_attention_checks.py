@@ -168,3 +168,16 @@ def test_row_splits():
     from tensorflow_graphics_point_clouds_amd import pc
     cloud = pc.PointCloud(torch.zeros(9, 3), sizes=torch.tensor([4, 0, 5]))
     assert attention.row_splits(cloud).tolist() == [0, 4, 4, 9] and attention.row_splits(cloud).dtype == _I32
+
+
+def test_row_splits_refuse_clouds_that_are_mixed():
+    from tensorflow_graphics_point_clouds_amd import pc
+    ordered = pc.PointCloud(torch.zeros(6, 3), batch_ids=torch.tensor([0, 0, 2, 2, 2, 3]), batch_size=5)
+    assert ordered.get_cloud_order() is None and attention.row_splits(ordered).tolist() == [0, 2, 2, 5, 6, 6]
+    mixed = pc.PointCloud(torch.zeros(6, 3), batch_ids=torch.tensor([1, 0, 1, 3, 0, 1]), batch_size=4)
+    assert mixed.get_cloud_order().tolist() == [1, 4, 0, 2, 5, 3]
+    with pytest.raises(_lib.InvalidArgumentError, match="cloud after cloud"):
+        attention.row_splits(mixed)
+    for cloud in (pc.PointCloud(torch.zeros(0, 3), batch_ids=torch.zeros(0), batch_size=2),
+                  pc.PointCloud(torch.zeros(2, 4, 3), sizes=torch.tensor([4, 1]))):
+        assert cloud.get_cloud_order() is None
