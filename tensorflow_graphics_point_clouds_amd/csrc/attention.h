@@ -233,9 +233,9 @@ __device__ __forceinline__ Frag<1> rest_frag(const v16f &s, int t, const F &...r
   return Frag<1>{{__builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]})}};
 }
 
-// Registers 8 t .. 8 t + 7 of a result as an operand.  One part: weights and score gradients are
-// rounded to bfloat16 here (their own product is rounded once to that type anyway; 2^-9 of a
-// weight); their sums and everything that the statistics are made of stay in float32.
+// Registers 8 t .. 8 t + 7 of a result as an operand.  One part: weights and logit gradients are
+// rounded to bfloat16 here, 2^-8 of each, and rest_frag has what that took from them for a
+// product of its own; their sums and everything that the statistics are made of stay in float32.
 template <int NP>
 __device__ __forceinline__ Frag<NP> result_frag(const v16f &s, int t) {
   const v4f lo = {s[8 * t], s[8 * t + 1], s[8 * t + 2], s[8 * t + 3]};

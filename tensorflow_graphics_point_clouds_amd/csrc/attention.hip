@@ -180,14 +180,15 @@ __global__ __launch_bounds__(kAttnThreads, (attn_forward_blocks_per_cu<T, DP, BI
           sum += p;
         }
       if constexpr (NP == 3) __builtin_amdgcn_s_setprio(1);
-      // A gradient will take D = do . o, and the row's logit gradients have to add up to zero: with
-      // bfloat16 weights rounded to one part, o is off by 2^-9 of its size, D with it, and rows of few
-      // keys got query gradients that were off by 1.5 %.  So then with the rest of the weights too.
-      // Behind a relative bias with that one's rest as well: gradients of its table are in float32,
-      // and they add up differences between o and the weights of 2^-18 over a bucket's pairs to 2 to
-      // 8e-6 of their size (with it 2e-7; 16 k causal tokens of 8 x 64 in 131 us instead of 123).
-      // (Operands of the values held for both products cost the third block of a compute unit, and one
-      // query over 4 x 200 k keys 145 us instead of 127.)
+      // bfloat16: with the rest of the weights too, which are then known to 2^-16 (one part alone, 2^-8,
+      // leaves outputs 2.4e-3 off instead of the 1.7e-3 of their own rounding, and D = do . o of the
+      // gradients with them).  Behind a relative bias with that one's rest as well: gradients of its
+      // table are in float32, and they add up differences between o and the weights over a bucket's
+      // pairs to 2 to 8e-6 of their size (with it 2e-7).  16 k causal tokens of 8 x 64 without a bias
+      // take 73, 88 us with one part and two, with a bias 86 and 115 with one and three; one query over
+      // 4 x 200 k keys 132 either way.  A call that a gradient will follow gives the same bits as
+      // one that none will.  (Operands of the values held for all parts: as fast or slower, 127 -> 145
+      // us where they cost the third block of a compute unit.)
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -197,17 +198,15 @@ __global__ __launch_bounds__(kAttnThreads, (attn_forward_blocks_per_cu<T, DP, BI
           for (int d = 0; d < DP / 32; ++d)
             acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), p, acc[d]);
           if constexpr (NP == 1) {
-            if (out_low) {
-              const Frag<NP> rest = rest_frag(s[u], t, p);
+            const Frag<NP> rest = rest_frag(s[u], t, p);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+              acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), rest, acc[d]);
+            if constexpr (BIAS != 0) {
+              const Frag<NP> last = rest_frag(s[u], t, p, rest);
 #pragma unroll
               for (int d = 0; d < DP / 32; ++d)
-                acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), rest, acc[d]);
-              if constexpr (BIAS != 0) {
-                const Frag<NP> last = rest_frag(s[u], t, p, rest);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
-                  acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), last, acc[d]);
-              }
+                acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), last, acc[d]);
             }
           }
         }

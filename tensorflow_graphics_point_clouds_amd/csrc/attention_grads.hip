@@ -233,6 +233,12 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d)
             acc[d] = mma<NP>(KTile::operand_t(kt, 32 * u + 16 * t, d), grads, acc[d]);
+          if constexpr (NP == 1) {             // (in two parts, known to 2^-16, as the weights)
+            const Frag<NP> rest = rest_frag(s, t, grads);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+              acc[d] = mma<NP>(KTile::operand_t(kt, 32 * u + 16 * t, d), rest, acc[d]);
+          }
         }
         __builtin_amdgcn_s_setprio(0);
       }
@@ -486,13 +492,33 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
           if (!key_ok || 32 * u + result_row(r) < limit) s[r] = dp[r] = 0.0f;
       }
       __builtin_amdgcn_s_setprio(1);
+      if constexpr (NP == 1) {
+        // weights and logit gradients in two parts, known to 2^-16; one sum after the other, which leaves
+        // the weights' registers free for the second (both at once: 34 registers spilled with 128 channels)
+        auto add = [&](const v16f &x, const __bf16 *tile, v16f *acc) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const Frag<NP> weights = result_frag<NP>(s, t), grads = result_frag<NP>(dp, t);
+          for (int t = 0; t < 2; ++t) {
+            const Frag<NP> part = result_frag<NP>(x, t);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          acc_v[d] = mma<NP>(QTile::operand_t(dt, 32 * u + 16 * t, d), weights, acc_v[d]);
-          acc_k[d] = mma<NP>(QTile::operand_t(qt, 32 * u + 16 * t, d), grads, acc_k[d]);
+            for (int d = 0; d < DP / 32; ++d)
+              acc[d] = mma<NP>(QTile::operand_t(tile, 32 * u + 16 * t, d), part, acc[d]);
+            const Frag<NP> rest = rest_frag(x, t, part);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+              acc[d] = mma<NP>(QTile::operand_t(tile, 32 * u + 16 * t, d), rest, acc[d]);
+          }
+        };
+        add(s, dt, acc_v);
+        add(dp, qt, acc_k);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const Frag<NP> weights = result_frag<NP>(s, t), grads = result_frag<NP>(dp, t);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            acc_v[d] = mma<NP>(QTile::operand_t(dt, 32 * u + 16 * t, d), weights, acc_v[d]);
+            acc_k[d] = mma<NP>(QTile::operand_t(qt, 32 * u + 16 * t, d), grads, acc_k[d]);
+          }
         }
       }
       __builtin_amdgcn_s_setprio(0);
