@@ -602,20 +602,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_offset_sums_kernel(int64_t 
   }
 }
 
-// Sums per bucket: a wavefront per (axis, bucket, head) over the offsets of the axis.
+// Sums per bucket: a wavefront per (axis, bucket, head) over the offsets of the axis.  (64-bit indices:
+// nothing bounds the buckets of a table.)
+constexpr int64_t kBucketBlocks = 1 << 20;
 __global__ __launch_bounds__(kAttnThreads) void attn_bucket_sums_kernel(int axes, int num_buckets, int heads,
                                                                         int width, const int *__restrict__ buckets,
                                                                         const double *__restrict__ in,
                                                                         float *__restrict__ dtable) {
-  const int i = blockIdx.x * (kAttnThreads / kWave) + threadIdx.x / kWave;
-  if (i >= axes * num_buckets * heads) return;
-  const int head = i % heads, bucket = (i / heads) % num_buckets, axis = i / heads / num_buckets;
-  double s = 0.0;
-  for (int o = lane_id(); o < width; o += kWave)
-    if (buckets[o] == bucket) s += in[((int64_t)head * axes + axis) * width + o];
+  constexpr int kWaves = kAttnThreads / kWave;
+  const int64_t n = (int64_t)axes * num_buckets * heads;
+  for (int64_t i = (int64_t)blockIdx.x * kWaves + threadIdx.x / kWave; i < n; i += (int64_t)gridDim.x * kWaves) {
+    const int head = (int)(i % heads), bucket = (int)(i / heads % num_buckets), axis = (int)(i / heads / num_buckets);
+    double s = 0.0;
+    for (int o = lane_id(); o < width; o += kWave)
+      if (buckets[o] == bucket) s += in[((int64_t)head * axes + axis) * width + o];
 #pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-  if (lane_id() == 0) dtable[i] = (float)s;
+    for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    if (lane_id() == 0) dtable[i] = (float)s;
+  }
 }
 
 
@@ -708,9 +712,9 @@ int launch_grads(hipStream_t s, AttnBatch b, const GradPlan &p, const void *out,
     const dim3 grid(blocks_for(per_head, 16), (unsigned)b.heads);
     attn_offset_sums_kernel<<<grid, kAttnThreads, 0, s>>>(b.num_q > 0 ? p.grad_blocks : 0, per_head, offsets, sums);
     MCCNN_LAUNCH_CHECK();
-    attn_bucket_sums_kernel<<<blocks_for((int64_t)b.axes * b.num_buckets * b.heads, kAttnThreads / kWave),
-                              kAttnThreads, 0, s>>>(b.axes, b.num_buckets, b.heads, 2 * b.max_offset + 1, b.buckets,
-                                                    sums, dtable);
+    const int64_t blocks = ((int64_t)b.axes * b.num_buckets * b.heads + kAttnThreads / kWave - 1) / (kAttnThreads / kWave);
+    attn_bucket_sums_kernel<<<(unsigned)(blocks < kBucketBlocks ? blocks : kBucketBlocks), kAttnThreads, 0, s>>>(
+        b.axes, b.num_buckets, b.heads, 2 * b.max_offset + 1, b.buckets, sums, dtable);
     MCCNN_LAUNCH_CHECK();
   }
   return MCCNN_OK;

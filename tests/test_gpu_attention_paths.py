@@ -187,3 +187,22 @@ def test_layer_norm_on_another_stream_and_in_a_graph(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+def test_gradient_of_a_table_beyond_32_bit_entries():
+    """2^31 entries (8 GB), of which eight buckets are used: theirs as of a small table, zeros elsewhere."""
+    from tensorflow_graphics_point_clouds_amd import attention
+    heads, many = 128, 1 << 24
+    q, k, v, g = _inputs(torch.float32, 20, 20, heads, 1, 8)
+    small, buckets = _table(1, 8, heads), attention.offset_buckets(8, 9)
+    last = (buckets + (many - 8)).int()              # the same buckets at the end of the large table
+    grads = []
+    for table, index in ((small, buckets), (torch.zeros(1, many, heads, device="cuda"), last)):
+        if index is last:
+            table[:, -8:] = small
+        table.requires_grad_()
+        out = attention.packed_attention(q, k, v, bias_table=table, bias_buckets=index)
+        grads += torch.autograd.grad(out, table, g)
+        del table, out
+    assert torch.equal(grads[1][:, -8:], grads[0])
+    assert not grads[1][:, :-8].any()
