@@ -11,6 +11,10 @@ from . import _lib
 
 _I32 = torch.int32
 
+# Offsets of a bias over all its axes, axes * (2 R + 1), that the kernels' shared memory has room for
+# (MCCNN_ATTENTION_MAX_OFFSETS).
+MAX_OFFSETS = 1344
+
 
 def layer_norm(features, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of `features` (float32 or
@@ -36,7 +40,8 @@ def packed_attention(queries, keys, values, query_splits=None, key_splits=None, 
     scale       of the products, 1 / sqrt(channels) by default
     bias_table  float32 [axes, buckets, heads], one to three axes: added to a logit is the sum over
                 the axes of the entry of bucket bias_buckets[offset + R], the offset key position -
-                query position clamped to -R .. R; `bias_buckets` int32 [2 R + 1] (`offset_buckets`)
+                query position clamped to -R .. R; `bias_buckets` int32 [2 R + 1] (`offset_buckets`),
+                axes * (2 R + 1) at most MAX_OFFSETS
     query_positions, key_positions  int32 [Nq, axes], [Nk, axes], for instance grid cells; without
                 them (one axis) the places of the tokens, counted as for `causal`
 
@@ -51,7 +56,8 @@ def offset_buckets(num_buckets, max_offset, bidirectional=True, device="cuda"):
     """Bucket of every offset -max_offset .. max_offset, int32 [2 * max_offset + 1]: the first half of
     a direction's buckets hold one offset each, the others grow by equal ratios up to `max_offset`.
     Bidirectional: the upper half of the buckets is for offsets above 0; otherwise those share
-    bucket 0 with offset 0.  (Whole-number arithmetic: no offset depends on a logarithm's last bit.)"""
+    bucket 0 with offset 0.  `packed_attention` takes at most MAX_OFFSETS offsets over all axes of a bias.
+    (Whole-number arithmetic: no offset depends on a logarithm's last bit.)"""
     side = num_buckets // 2 if bidirectional else num_buckets
     near = side // 2
     if near < 1 or max_offset < near:

@@ -294,12 +294,16 @@ class LayerNorm(torch.nn.Module):
 
 class RelativeBias(torch.nn.Module):
     """A learned bias of attention logits per head, axis and bucket of the relative position: the
-    place in the cloud (one axis, no positions) or integer positions such as grid cells.  Starts
-    at zero."""
+    place in the cloud (one axis, no positions) or integer positions such as grid cells; num_axes *
+    (2 max_offset + 1) at most `attention.MAX_OFFSETS`.  Starts at zero."""
 
     def __init__(self, num_heads, num_buckets=32, max_offset=128, num_axes=1, bidirectional=True,
                  device="cuda"):
         super().__init__()
+        if num_axes * (2 * max_offset + 1) > attention.MAX_OFFSETS:
+            raise _lib.InvalidArgumentError(
+                "RelativeBias expects at most %d offsets over all axes, got %d times %d" %
+                (attention.MAX_OFFSETS, num_axes, 2 * max_offset + 1))
         self.table = torch.nn.Parameter(torch.zeros((num_axes, num_buckets, num_heads), dtype=_F32,
                                                     device=device))
         self.register_buffer("buckets", attention.offset_buckets(num_buckets, max_offset,

@@ -29,7 +29,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kAttnThreads = 256;
 constexpr int kAttnRows = 128;            // query rows (or keys) of a block, 32 per wavefront
 constexpr int kAttnMaxDim = 128;
-constexpr int kAttnMaxOffsets = 1344;     // axes * (2 R + 1): what the LDS has room for
+constexpr int kAttnMaxOffsets = MCCNN_ATTENTION_MAX_OFFSETS;   // axes * (2 R + 1): what the LDS has room for
 
 // A packed batch as the kernels see it.  Strides are in elements; the innermost one is 1.
 struct AttnBatch {

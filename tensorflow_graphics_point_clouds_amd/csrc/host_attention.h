@@ -263,6 +263,9 @@ Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
                std::to_string(q.size(1)) + " heads");
     expect(buckets.dim() == 1 && buckets.size(0) % 2 == 1 && buckets.size(0) <= (1 << 24),
            "packed_attention expects buckets of the offsets -R to R, got " + shape_of(buckets));
+    expect(table.size(0) * buckets.size(0) <= MCCNN_ATTENTION_MAX_OFFSETS,
+           "packed_attention expects a bias of at most " + std::to_string(MCCNN_ATTENTION_MAX_OFFSETS) +
+               " offsets over all axes, got " + std::to_string(table.size(0)) + " times " + std::to_string(buckets.size(0)));
     expect(q_pos.defined() || table.size(0) == 1,
            "packed_attention expects positions for a bias of " + std::to_string(table.size(0)) + " axes");
     for (const auto &side : {std::make_pair(q_pos, q), std::make_pair(k_pos, k)})
