@@ -1094,7 +1094,8 @@ int mccnn_layer_norm_grads(mccnn_stream_t stream, int dtype, int64_t num_rows, i
  * The optional relative bias is the sum over its axes a of
  *   table[a, buckets[clamp(k_pos[j, a] - q_pos[i, a], -max_offset, max_offset) + max_offset], head],
  * without positions for one axis with a token's place among the keys of its cloud as position.
- * It has at most MCCNN_ATTENTION_MAX_OFFSETS offsets over all axes, axes * (2 * max_offset + 1).  A bucket outside [0, num_buckets) adds nothing.
+ * It has at most MCCNN_ATTENTION_MAX_OFFSETS offsets over all axes, axes * (2 * max_offset + 1).
+ * A bucket outside [0, num_buckets) adds nothing.
  * Splits are row offsets [clouds + 1] from 0 to the number of rows; rows outside every cloud look
  * at nothing.  The innermost stride of q, k and v is 1; the others are given in elements. */
 typedef struct mccnn_attention {

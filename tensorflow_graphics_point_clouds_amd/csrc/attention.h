@@ -427,9 +427,12 @@ __device__ __forceinline__ bool find_work(const AttnBatch &b, int t, bool revers
 
 // A bias in units of log 2.  Masks are written as the type's lowest value, which has none: everything
 // below -6.9e37 becomes -1e38, three of which still add up to a finite logit, so that a row with
-// nothing but such entries is the mean of its values, as it is in natural units.  -inf stays.
+// nothing but such entries is the mean of its values, as it is in natural units; the largest values
+// likewise.  Infinities and NaN stay.
 __device__ __forceinline__ float log2_units(float bias) {
-  return bias == -INFINITY ? bias : fmaxf(bias * kLog2e, -1.0e38f);
+  const float x = bias * kLog2e;
+  if (bias == INFINITY || bias == -INFINITY) return bias;
+  return x > 1.0e38f ? 1.0e38f : x < -1.0e38f ? -1.0e38f : x;
 }
 
 // table[a, bucket(o - R), head0 + g] in units of log 2 for all offsets o, as [g][a][2 R + 1] in LDS.

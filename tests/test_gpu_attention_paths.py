@@ -206,3 +206,28 @@ def test_gradient_of_a_table_beyond_32_bit_entries():
         del table, out
     assert torch.equal(grads[1][:, -8:], grads[0])
     assert not grads[1][:, :-8].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("places", [True, False])
+def test_table_entries_that_are_no_ordinary_numbers(dtype, places):
+    """NaN reaches the rows that meet its bucket (it is no mask), and no others; the largest finite value
+    leaves a row the mean of the values that have it, as the lowest hides them."""
+    from tensorflow_graphics_point_clouds_amd import attention
+    q, k, v, g = _inputs(dtype, 90, 90, 2, 2, 32)
+    buckets, table = attention.offset_buckets(8, 12), _table(1, 8, 2)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    pos = None if places else torch.randint(0, 20, (90, 1), device="cuda", generator=gen, dtype=torch.int32)
+    offset = torch.arange(90, device="cuda")[None] - torch.arange(90, device="cuda")[:, None] if places else \
+        pos[None, :, 0] - pos[:, None, 0]
+    index = buckets[(offset.clamp(-12, 12) + 12).long()]
+    bad = table.clone()
+    bad[0, 7, 1] = math.nan
+    out = attention.packed_attention(q, k, v, bias_table=bad, bias_buckets=buckets, query_positions=pos, key_positions=pos)
+    met = (index == 7).any(1)
+    assert met.any() and not met.all()
+    assert torch.equal(torch.isnan(out[:, 1]).all(1), met) and torch.equal(torch.isnan(out[:, 1]).any(1), met)
+    assert torch.isfinite(out[:, 0]).all()
+    table[0, 5] = 3.4028234663852886e38
+    got = _run(q, k, v, g, [0, 90], [0, 90], table=table, buckets=buckets, qpos=pos, kpos=pos)
+    assert all(torch.isfinite(t).all() for t in got)
