@@ -74,7 +74,13 @@ inline int attn_pack(const AttnBatch &b, int room) {
 inline int64_t attn_places(int64_t rows, int clouds) { return rows / kAttnRows + clouds + 2; }
 // Block id = (place * parts + part) * columns + column: the columns (heads) of a piece go to
 // neighbouring XCDs, so that each of the eight L2 sees few heads' keys.
-constexpr int64_t kAttnMaxBlocks = (1 << 24) - 1;     // of 256 threads: a grid counts them in 32 bits
+// A grid counts the threads of a dimension in 32 bits: blocks behind the first 2^24 - 1 of 256 take a
+// second row of it, whose last ones may lie behind the last place.
+constexpr int64_t kAttnRowBlocks = (1 << 24) - 1, kAttnMaxBlocks = ((int64_t)1 << 31) - 1;
+inline dim3 attn_grid(int64_t blocks) {
+  const int64_t row = blocks < kAttnRowBlocks ? blocks : kAttnRowBlocks;
+  return dim3((unsigned)row, (unsigned)((blocks + row - 1) / row));
+}
 // Parts that a long axis is cut into, none with less than about 256 of its elements.  Blocks of full
 // rows are bound by their arithmetic: as many as are at work at a time, two per compute unit, twice as
 // many under a causal mask, whose walks differ (key gradients of 13 001 tokens, 404 blocks: 1301 us in
@@ -127,6 +133,8 @@ constexpr int attn_tile_rows() {
 }
 
 #ifdef __HIPCC__
+
+__device__ __forceinline__ unsigned attn_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));

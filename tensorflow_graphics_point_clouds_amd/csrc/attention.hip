@@ -33,8 +33,8 @@ __global__ __launch_bounds__(kAttnThreads, (attn_forward_blocks_per_cu<T, DP, BI
   int *kpos = reinterpret_cast<int *>(ktile + 4 * KTile::kElems);      // [2][3][KT]
   float *table = reinterpret_cast<float *>(kpos + (BIAS == 2 ? 6 * KT : 0));
 
-  const int columns = b.heads / b.pack, column = blockIdx.x % columns, place = blockIdx.x / columns / parts;
-  const int part = blockIdx.x / columns % parts;
+  const unsigned block = attn_block(), columns = b.heads / b.pack;
+  const int column = block % columns, place = block / columns / parts, part = block / columns % parts;
   CloudWork work;
   if (!find_work<false>(b, place, b.causal, work)) return;
   const int num_q = work.num_q, shift = work.used - num_q;
@@ -346,8 +346,8 @@ int launch_forward(hipStream_t s, const AttnBatch &b, const ForwardPlan &p, void
                 (long long)b.num_q, b.heads);
   float *part_out = reinterpret_cast<float *>(ws + p.part_out);
   float *part_max = reinterpret_cast<float *>(ws + p.part_max), *part_sum = reinterpret_cast<float *>(ws + p.part_sum);
-  kernel<<<(unsigned)grid, kAttnThreads, lds, s>>>(b, p.parts, static_cast<T *>(out), out_low, part_out,
-                                         p.parts > 1 ? part_max : row_max, p.parts > 1 ? part_sum : row_sum);
+  kernel<<<attn_grid(grid), kAttnThreads, lds, s>>>(b, p.parts, static_cast<T *>(out), out_low, part_out,
+                                          p.parts > 1 ? part_max : row_max, p.parts > 1 ? part_sum : row_sum);
   MCCNN_LAUNCH_CHECK();
   if (p.parts > 1) {
     const int64_t rows = b.num_q * b.heads;

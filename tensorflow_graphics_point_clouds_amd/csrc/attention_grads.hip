@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
     AttnBatch b, int parts, const T *__restrict__ out, const float *__restrict__ out_low,
     const T *__restrict__ dout, const float *__restrict__ row_max, const float *__restrict__ row_sum,
     float *__restrict__ delta, T *__restrict__ dq, float *__restrict__ part_dq,
-    float *__restrict__ offset_grads, int copies_log2) {
+    float *__restrict__ offset_grads, int grad_blocks, int copies_log2) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   constexpr int KT = attn_tile_rows<T, DP>();
   constexpr int SUB = KT / 32;
@@ -50,15 +50,16 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
   // [4][pack][axes][width][copies]
   double *sums = reinterpret_cast<double *>(table + ((b.pack * per_head + 1) & ~1));
 
-  const int columns = b.heads / b.pack, column = blockIdx.x % columns, grad_block = blockIdx.x / columns;
+  const unsigned block = attn_block(), columns = b.heads / b.pack;
+  const int column = block % columns, grad_block = block / columns;
+  if (grad_block >= grad_blocks) return;               // (behind the last place)
   const int place = grad_block / parts, part = grad_block % parts;
   const int head0 = column * b.pack, kv_head = head0 / (b.heads / b.kv_heads);
-  const int64_t grad_blocks = gridDim.x / columns;
   CloudWork work;
   if (!find_work<false>(b, place, b.causal, work)) {
     if (BIAS && offset_grads)
       for (int i = threadIdx.x; i < b.pack * per_head; i += kAttnThreads)
-        offset_grads[((head0 + i / per_head) * grad_blocks + grad_block) * per_head + i % per_head] = 0.0f;
+        offset_grads[((int64_t)(head0 + i / per_head) * grad_blocks + grad_block) * per_head + i % per_head] = 0.0f;
     return;
   }
   const int num_q = work.num_q, shift = work.used - num_q;
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
         double total = 0.0;
         for (int w = 0; w < 4; ++w)
           for (int c = 0; c < copies; ++c) total += sums[(w * n + i) * copies + c];
-        offset_grads[((head0 + i / per_head) * grad_blocks + grad_block) * per_head + i % per_head] = (float)total;
+        offset_grads[((int64_t)(head0 + i / per_head) * grad_blocks + grad_block) * per_head + i % per_head] = (float)total;
       }
     }
   }
@@ -317,8 +318,8 @@ __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void a
   int *qposs = reinterpret_cast<int *>(stats + 6 * QT);                 // [2][3][QT]
   float *table = reinterpret_cast<float *>(qposs + (BIAS == 2 ? 6 * QT : 0));
 
-  const int column = blockIdx.x % b.kv_heads, place = blockIdx.x / b.kv_heads / parts;
-  const int part = blockIdx.x / b.kv_heads % parts;
+  const unsigned block = attn_block();
+  const int column = block % b.kv_heads, place = block / b.kv_heads / parts, part = block / b.kv_heads % parts;
   CloudWork work;
   if (!find_work<true>(b, place, false, work)) return;
   const int num_q = work.num_q, shift = work.used - num_q;
@@ -678,9 +679,9 @@ int launch_grads(hipStream_t s, AttnBatch b, const GradPlan &p, const void *out,
     const int64_t grid = p.grad_blocks * (b.heads / b.pack);
     MCCNN_REQUIRE(grid <= kAttnMaxBlocks, "attention gradients of %lld queries and %d heads take too many blocks",
                   (long long)b.num_q, b.heads);
-    kernel<<<(unsigned)grid, kAttnThreads, lds, s>>>(b, p.q_parts, static_cast<const T *>(out), out_low,
+    kernel<<<attn_grid(grid), kAttnThreads, lds, s>>>(b, p.q_parts, static_cast<const T *>(out), out_low,
                                            static_cast<const T *>(dout), row_max, row_sum, delta, static_cast<T *>(dq),
-                                           at(p.part_q), offsets, copies_log2);
+                                           at(p.part_q), offsets, (int)p.grad_blocks, copies_log2);
     MCCNN_LAUNCH_CHECK();
     if (p.q_parts > 1) {
       const int64_t n = b.num_q * b.heads * b.dim;
@@ -698,7 +699,7 @@ int launch_grads(hipStream_t s, AttnBatch b, const GradPlan &p, const void *out,
     const int64_t grid = attn_places(b.num_k, b.clouds) * b.kv_heads * p.k_parts;
     MCCNN_REQUIRE(grid <= kAttnMaxBlocks, "attention gradients of %lld keys and %d heads take too many blocks",
                   (long long)b.num_k, b.kv_heads);
-    kernel<<<(unsigned)grid, kAttnThreads, lds, s>>>(b, p.k_parts, static_cast<const T *>(dout), row_max, row_sum, delta,
+    kernel<<<attn_grid(grid), kAttnThreads, lds, s>>>(b, p.k_parts, static_cast<const T *>(dout), row_max, row_sum, delta,
                                            static_cast<T *>(dk), static_cast<T *>(dv), at(p.part_k), at(p.part_v));
     MCCNN_LAUNCH_CHECK();
     if (p.k_parts > 1) {
