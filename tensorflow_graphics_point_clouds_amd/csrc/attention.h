@@ -227,15 +227,12 @@ __device__ __forceinline__ v2f widen_pair(const Frag<1> &f, int e) {
   const unsigned pair = u[e];             // (a bit cast of u[e] itself takes element 0 every time)
   return widen2(__builtin_bit_cast(v2bf, pair));
 }
-// What one rounding to one part, or a second one of the rest, has left of registers
-// 8 t .. 8 t + 7, as an operand.
-template <typename... F>
-__device__ __forceinline__ Frag<1> rest_frag(const v16f &s, int t, const F &...rounded) {
+// What the rounding to one part has left of registers 8 t .. 8 t + 7, as an operand.
+__device__ __forceinline__ Frag<1> rest_frag(const v16f &s, int t, const Frag<1> &rounded) {
   unsigned w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    v2f x = v2f{s[8 * t + 2 * e], s[8 * t + 2 * e + 1]};
-    ((x = x - widen_pair(rounded, e)), ...);
+    const v2f x = v2f{s[8 * t + 2 * e], s[8 * t + 2 * e + 1]} - widen_pair(rounded, e);
     w[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, v2bf));
   }
   return Frag<1>{{__builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]})}};
@@ -259,6 +256,36 @@ __device__ __forceinline__ Frag<NP> result_frag(const v16f &s, int t) {
     }
     return Frag<1>{{__builtin_bit_cast(v8bf, v4u{w[0], w[1], w[2], w[3]})}};
   }
+}
+
+// Registers 8 t .. 8 t + 7 of softmax weights as P operands, the leading bits, the following ones and at
+// last the rounded rest: 2^-15 of a weight is left out of two, nothing of three.  All parts are above 0
+// (2^-126 at least where nothing is left; cut off, not rounded, so that no rest is negative): a value of
+// infinity, which each of them multiplies, then stays one.
+template <int P>
+__device__ __forceinline__ void weight_parts(const v16f &s, int t, Frag<1> *parts) {
+  typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+  constexpr unsigned kTop = 0xffff0000u;
+  unsigned w[P][4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a = s[8 * t + 2 * e], b = s[8 * t + 2 * e + 1];
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      unsigned u;
+      if (q + 1 < P) {
+        u = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   // both upper halves
+        a -= __uint_as_float(__float_as_uint(a) & kTop);
+        b -= __uint_as_float(__float_as_uint(b) & kTop);
+      } else {
+        u = __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{a, b}, v2bf));
+      }
+      if (q > 0) u = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(v2us, u), v2us{0x80, 0x80}));
+      w[q][e] = u;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < P; ++q) parts[q] = Frag<1>{{__builtin_bit_cast(v8bf, v4u{w[q][0], w[q][1], w[q][2], w[q][3]})}};
 }
 
 // The sum of the products of eight values with eight others, in float32.

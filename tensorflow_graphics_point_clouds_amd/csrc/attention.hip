@@ -180,35 +180,27 @@ __global__ __launch_bounds__(kAttnThreads, (attn_forward_blocks_per_cu<T, DP, BI
           sum += p;
         }
       if constexpr (NP == 3) __builtin_amdgcn_s_setprio(1);
-      // bfloat16: with the rest of the weights too, which are then known to 2^-16 (one part alone, 2^-8,
-      // leaves outputs 2.4e-3 off instead of the 1.7e-3 of their own rounding, and D = do . o of the
-      // gradients with them).  Behind a relative bias with that one's rest as well: gradients of its
-      // table are in float32, and they add up differences between o and the weights over a bucket's
-      // pairs to 2 to 8e-6 of their size (with it 2e-7).  16 k causal tokens of 8 x 64 without a bias
-      // take 73, 88 us with one part and two, with a bias 86 and 115 with one and three; one query over
-      // 4 x 200 k keys 132 either way.  A call that a gradient will follow gives the same bits as
-      // one that none will.  (Operands of the values held for all parts: as fast or slower, 127 -> 145
-      // us where they cost the third block of a compute unit.)
+      // bfloat16 weights in two parts, known to 2^-15 (one part alone, 2^-8, left outputs 2.4e-3 off instead
+      // of the 1.66e-3 of their own rounding, and D = do . o of the gradients with them).  Behind a relative
+      // bias in three: gradients of its table are in float32, and they add up differences between o and
+      // the weights over a bucket's pairs to 2 to 8e-6 of their size (with three 2e-7).  16 k causal
+      // tokens of 8 x 64 without a bias take 74 us with one part and 90 with two, with a bias 86 with one
+      // and 122 with three; one query over 4 x 200 k keys 133 and 136.  A call that a gradient will
+      // follow gives the same bits as one that none will.  (Operands of the values held for all parts:
+      // as fast or slower, 127 -> 145 us where they cost the third block of a compute unit.)
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const Frag<NP> p = result_frag<NP>(s[u], t);
+          constexpr int P = NP == 3 ? 1 : BIAS ? 3 : 2;
+          Frag<NP> p[P];
+          if constexpr (NP == 3) p[0] = result_frag<NP>(s[u], t);
+          else weight_parts<P>(s[u], t, p);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d)
-            acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), p, acc[d]);
-          if constexpr (NP == 1) {
-            const Frag<NP> rest = rest_frag(s[u], t, p);
+          for (int q = 0; q < P; ++q)
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
-              acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), rest, acc[d]);
-            if constexpr (BIAS != 0) {
-              const Frag<NP> last = rest_frag(s[u], t, p, rest);
-#pragma unroll
-              for (int d = 0; d < DP / 32; ++d)
-                acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), last, acc[d]);
-            }
-          }
+              acc[d] = mma<NP>(KTile::operand_t(vt, 32 * u + 16 * t, d), p[q], acc[d]);
         }
       if constexpr (NP == 3) __builtin_amdgcn_s_setprio(0);
     }
