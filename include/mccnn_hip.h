@@ -1090,7 +1090,10 @@ int mccnn_layer_norm_grads(mccnn_stream_t stream, int dtype, int64_t num_rows, i
  * where j runs over the keys of the query's cloud that are there (k_sizes), that the mask keeps and,
  * if causal, that do not lie behind the query; the last query stands at the last key.  A query
  * that nothing is left for gets zeros.  Keys that are masked or not there may hold anything; keys
- * hidden by causality only have to be finite.
+ * hidden by causality only have to be finite.  Logits, statistics and sums are in float32; 16-bit
+ * results are rounded once.  A value of infinity that is looked at gives infinity with 16-bit
+ * features; float32 operands are multiplied in three parts of 16 bits, and an infinity in one, or
+ * a number within 2^-8 of the largest, gives NaN wherever it is looked at.
  * The optional relative bias is the sum over its axes a of
  *   table[a, buckets[clamp(k_pos[j, a] - q_pos[i, a], -max_offset, max_offset) + max_offset], head],
  * without positions for one axis with a token's place among the keys of its cloud as position.

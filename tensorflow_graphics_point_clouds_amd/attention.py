@@ -41,12 +41,18 @@ def packed_attention(queries, keys, values, query_splits=None, key_splits=None, 
     bias_table  float32 [axes, buckets, heads], one to three axes: added to a logit is the sum over
                 the axes of the entry of bucket bias_buckets[offset + R], the offset key position -
                 query position clamped to -R .. R; `bias_buckets` int32 [2 R + 1] (`offset_buckets`),
-                axes * (2 R + 1) at most MAX_OFFSETS
+                axes * (2 R + 1) at most MAX_OFFSETS.  -inf hides a bucket
     query_positions, key_positions  int32 [Nq, axes], [Nk, axes], for instance grid cells; without
                 them (one axis) the places of the tokens, counted as for `causal`
 
     A query that nothing is left for gets zeros and zero gradients.  Differentiable (once) in
-    queries, keys, values and bias_table; gradients of keys that are not looked at are zero."""
+    queries, keys, values and bias_table; gradients of keys that are not looked at are zero.
+
+    Everything between operands and results is float32 (bfloat16 weights are multiplied in parts), and
+    a call that records a gradient gives the same bits as one that does not.  Keys hidden by `causal`
+    alone have to be finite.  A value of infinity that is looked at gives infinity in bfloat16; in
+    float32 an infinity that is looked at, or a number within 2^-8 of the largest, gives NaN (such
+    operands are multiplied as three bfloat16 parts)."""
     return _lib.host().packed_attention(queries, keys, values, query_splits, key_splits, key_sizes,
                                         key_mask, causal, scale, bias_table, bias_buckets,
                                         query_positions, key_positions)

@@ -83,10 +83,10 @@ inline dim3 attn_grid(int64_t blocks) {
 }
 // Parts that a long axis is cut into, none with less than about 256 of its elements.  Blocks of full
 // rows are bound by their arithmetic: as many as are at work at a time, two per compute unit, twice as
-// many under a causal mask, whose walks differ (key gradients of 13 001 tokens, 404 blocks: 1301 us in
-// one part, 732 in two).  Blocks of few rows wait for memory: `few`,
-// three per compute unit (one query per cloud over 4 x 200 k keys of 64 bfloat16 channels 233, 134, 128,
-// 143 us with 256, 512, 768, 1024 blocks), in a forward pass of up to 32 channels four.
+// many under a causal mask, whose walks differ (13 001 tokens, whose key gradients are 404 blocks: a
+// training pass of 1761 us with those in one part, 1391 in two).  Blocks of few rows wait for memory:
+// `few`, three per compute unit (one query per cloud over 4 x 200 k keys of 64 bfloat16 channels 256, 145,
+// 134, 149 us with 256, 512, 768, 1024 blocks), in a forward pass of up to 32 channels four.
 inline int attn_parts(int64_t rows, int clouds, int64_t columns, int64_t axis, bool causal, int few = 768) {
   const int64_t full = rows / kAttnRows, blocks = (full > clouds ? full : clouds) * columns;
   const int64_t want = (full <= clouds ? few : causal ? 1024 : 512) / (blocks > 0 ? blocks : 1);
@@ -118,9 +118,9 @@ constexpr int attn_blocks_per_cu() {
   return sizeof(T) == 4 && DP > 64 ? 1 : 2;
 }
 // The same of the forward pass: with up to 64 bfloat16 channels three blocks fit, all but a few
-// registers of a lane with a bias of token offsets (8 x 2000 tokens, weights in two parts: 132 -> 117
-// us; with positions 28 to 38 of them would spill, and of the query gradients' 16, for 182 us instead
-// of 166).
+// registers of a lane with a bias of token offsets (8 x 2000 tokens forward: 130 us with three blocks and
+// 3 registers spilled, 138 with two; with positions 28 to 38 of them would spill, and of the query
+// gradients' 19, for a training pass of 466 us instead of 447).
 template <typename T, int DP, int BIAS>
 constexpr int attn_forward_blocks_per_cu() {
   return sizeof(T) == 2 && DP <= 64 && BIAS != 2 ? 3 : attn_blocks_per_cu<T, DP>();

@@ -15,11 +15,11 @@ constexpr float kSlack = 8.0f;
 // further) and a column of the transposed result.
 //
 // Bound, with full rows, by the matrix pipe and the exponentials beside it (per wavefront and 32 x 32
-// logits 32 cycles for each of the 48 float32 / 8 bfloat16 matrix instructions of 64 channels, some
-// 300 / 150 vector instructions of 4 and 16 exponentials of 16): 8 x 4096 tokens of 4 x 64 float32 in
-// 727 us are 189 TFLOP/s, six times that on the bf16 pipe; of 4 x 128 bfloat16 in 340 us 808.  With a
-// query per cloud by memory: 4 x 200 k keys, 655 MB in 127 us.  Small batches by a block's walk: 5 us
-// for an empty one, 1.5 us per tile.
+// logits 32 cycles for each of the 48 float32 / 12 bfloat16 matrix instructions of 64 channels, some
+// 300 / 200 vector instructions of 4 and 16 exponentials of 16): 8 x 4096 tokens of 4 x 64 float32 in
+// 684 us are 201 TFLOP/s, six times that on the bf16 pipe; of 4 x 128 bfloat16 in 407 us 675, half as
+// much again on the pipe.  With a query per cloud by memory: 4 x 200 k keys, 655 MB in 132 us.  Small
+// batches by a block's walk: 5 us for an empty one, 1.5 us per tile.
 template <typename T, int DP, int BIAS, bool VEC>
 __global__ __launch_bounds__(kAttnThreads, (attn_forward_blocks_per_cu<T, DP, BIAS>())) void attn_forward_kernel(
     AttnBatch b, int parts, T *__restrict__ out, float *__restrict__ out_low,
@@ -312,8 +312,8 @@ struct ForwardPlan {
 ForwardPlan forward_plan(AttnBatch &b) {
   ForwardPlan p{};
   b.pack = attn_pack(b, 8192);
-  // 768 and 1024 blocks of few rows, 32 channels: 4 x 200 k keys of two heads in float32 135 and 124 us, in
-  // bfloat16 64 and 61; 5 x 12 k keys of eight heads 46 and 39, 24.7 and 23.6.
+  // 768 and 1024 blocks of few rows, 32 channels: 4 x 200 k keys of two heads in float32 107 and 96 us, in
+  // bfloat16 60.8 and 60.4; 5 x 12 k keys of eight heads 45.7 and 44.8, 29.1 and 29.5.
   const int few = b.dim <= 32 && !b.axes ? 1024 : 768;
   p.parts = attn_parts(b.num_q * b.pack, b.clouds, b.heads / b.pack, b.num_k, b.causal, few);
   if (p.parts > 1) {

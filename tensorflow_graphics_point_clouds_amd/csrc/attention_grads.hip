@@ -21,13 +21,13 @@ __device__ __forceinline__ v16f zero16() {
 }
 
 // The wavefronts of a SIMD take turns at its matrix pipe: the one in the middle of its products goes
-// first (s_setprio), the other one's exponentials fill the gaps.  2 to 5 % in both passes, 7 % in the
-// float32 forward pass; the bfloat16 one gets 2 % slower with it and goes without.
+// first (s_setprio), the other one's exponentials fill the gaps.  1 to 6 % in both passes, 7 % in the
+// float32 forward pass; the bfloat16 one is between 2 % faster and 1 % slower with it and goes without.
 
 // Query gradients: three products per pair, 16 x 1024 points of 4 x 64 float32 in 158 us (163 TFLOP/s),
-// 4 x 3250 tokens causal of 16 x 128 bfloat16 in 387 (690).  A block as in the forward pass (128 rows,
-// one part of the keys).  D is formed here and left in `delta` for the other pass.  Where the bias has a
-// gradient every wavefront adds its logit gradients up per offset in an LDS table of its own (one
+// 4 x 3250 tokens causal of 16 x 128 bfloat16 in 419 (638; their logit gradients are multiplied in two
+// parts, a third more on the pipe).  A block as in the forward pass (128 rows, one part of the keys).
+// D is formed here and left in `delta` for the other pass.  Where the bias has a gradient every wavefront adds its logit gradients up per offset in an LDS table of its own (one
 // wavefront's additions to one address are served in lane order), and the block writes the sum of its
 // four.  The table is in 64 bits for the speed of it: an LDS addition of 64 floats takes 192 cycles of
 // the compute unit, whatever the addresses, one of 64 doubles 8 without conflicts and 33 into 32 random
@@ -294,10 +294,10 @@ constexpr bool attn_values_in_lds() {
   return sizeof(T) == 2 && DP == 128;
 }
 
-// Key and value gradients: four products per pair, the same batches in 198 us (174 TFLOP/s) and 560
-// (640): the matrix pipe, and with 128 channels LDS reads of as many cycles.  A block owns 128 keys (32
-// per wavefront, one per lane) of one cloud and key head and walks over the queries of all heads that
-// share them, or over one part of that walk.
+// Key and value gradients: four products per pair, the same batches in 198 us (174 TFLOP/s) and 634
+// (565, half as much again on the pipe): the matrix pipe, and with 128 channels LDS reads of as many
+// cycles.  A block owns 128 keys (32 per wavefront, one per lane) of one cloud and key head and walks
+// over the queries of all heads that share them, or over one part of that walk.
 template <typename T, int DP, int BIAS, bool VEC>
 __global__ __launch_bounds__(kAttnThreads, (attn_blocks_per_cu<T, DP>())) void attn_key_grads_kernel(
     AttnBatch b, int parts, const T *__restrict__ dout, const float *__restrict__ row_max,

@@ -285,3 +285,12 @@ def test_infinite_bfloat16_values_that_are_looked_at(bias, nq, nk):
         assert torch.isnan(out[..., 9]).all()
         others = [c for c in range(24) if c not in (3, 5, 9)]
         assert torch.equal(out[..., others], plain[..., others])
+
+
+def test_rows_without_any_cloud():
+    from tensorflow_graphics_point_clouds_amd import attention
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_() for t in _inputs(torch.float32, 300, 500, 4, 2, 16)[:3]]
+    out = attention.packed_attention(*leaves, none, none, causal=True)
+    assert out.shape == leaves[0].shape and not out.any()
+    assert not any(t.any() for t in torch.autograd.grad(out, leaves, torch.ones_like(out)))
