@@ -8,8 +8,9 @@
 // Logits are kept in units of log 2 (scale and biases times 1 / log 2), exponentials are powers of 2.
 //
 // All products are 32 x 32 x 16 steps of the bf16 matrix pipe with float32 accumulation.  bfloat16
-// operands are taken as they are (one part); float32 operands as three bfloat16 parts each, six
-// part products per step (split.h), which is as exact as float32 products.
+// operands are taken as they are (one part), softmax weights and logit gradients beside them in two or
+// three; float32 operands as three bfloat16 parts each, six part products per step (split.h), which
+// is as exact as float32 products.
 //
 // Layout of a 32 x 32 result in registers: lane l holds column l & 31, and its register r row
 // 8 (r / 4) + 4 (l >> 5) + r % 4.  Scores are formed with the reduction's other side in the rows
